@@ -1057,7 +1057,7 @@ class MasterWeightAdamW:
     `fused_clip` (GPU): norm, clipping and the conversion to float32 by optim.GradientClipper, with the norm's sums in float64."""
 
     def __init__(self, model, lr=1.41e-4, lr_backbone=1.41e-5, text_encoder_lr=1.41e-5, weight_decay=1e-4, fused_clip=False):
-        self.fused_clip, self._clipper = fused_clip, None
+        self.fused_clip = fused_clip
         named = [(n, p) for n, p in model.named_parameters() if p.requires_grad]
         self.names = [n for n, _ in named]
         self.params = [p for _, p in named]
@@ -1088,13 +1088,10 @@ class MasterWeightAdamW:
                 self.gbuf[i].zero_()
         if self.fused_clip and max_norm > 0 and have:
             grads, out = [self.params[i].grad for i in have], [self.gbuf[i] for i in have]
-            clipper = self._clipper
-            if clipper is None or len(clipper.tensors) != len(grads) or any(a is not b for a, b in zip(clipper.tensors, grads)):
-                # (a gradient in another element order than its float32 buffer, e.g. of a channels-last weight, is laid out as the buffer)
-                clipper = GradientClipper([g if _same_layout(g, o) else torch.empty_like(o, dtype=g.dtype).copy_(g)
-                                           for g, o in zip(grads, out)], out=out)
-                self._clipper = clipper if all(a is b for a, b in zip(clipper.tensors, grads)) else None
-            clipper.clip(max_norm)
+            # (laid out anew each step: gradients that were dropped, or whose memory was replaced, must not live on in it.  A gradient in
+            #  another element order than its float32 buffer, e.g. of a channels-last weight, is laid out as the buffer)
+            GradientClipper([g if _same_layout(g, o) else torch.empty_like(o, dtype=g.dtype).copy_(g) for g, o in zip(grads, out)],
+                            out=out).clip(max_norm)
         else:
             torch._foreach_copy_([self.gbuf[i] for i in have], [self.params[i].grad for i in have])
             if max_norm > 0:
