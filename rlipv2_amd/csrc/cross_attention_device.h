@@ -442,9 +442,9 @@ inline Plan plan_for(int64_t resident, int64_t streamed_tiles, int64_t groups, i
     // (half of the compute units have work already: joining pays from 16 tiles a split on -- 2331 rows of heads of 64 over 1091 keys
     // 24.6 us with one split, 30.5 with three)
     if (have >= 128 && least == 4) most = streamed_tiles / 16 > 1 ? streamed_tiles / 16 : 1;
-    const int64_t split = have ? 256 * (int64_t)fit / have : 1;
-    const int64_t fewest = (streamed_tiles + longest - 1) / longest;
-    p.splits = (int)(split < fewest ? (fewest < 1 ? 1 : fewest) : split > most ? (most < fewest ? fewest : most) : split);
+    const int64_t split = have ? 256 * (int64_t)fit / have : 1, fewest = streamed_tiles > longest ? (streamed_tiles + longest - 1) / longest : 1;
+    if (most < fewest) most = fewest;
+    p.splits = (int)(split < fewest ? fewest : split > most ? most : split);        // (one where nothing is streamed)
     return p;
 }
 
