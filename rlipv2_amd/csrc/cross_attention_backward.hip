@@ -327,6 +327,9 @@ __global__ __launch_bounds__(64 * NW, OCC) void key_kernel(cross_attention_args 
             ahead<AHEAD, 2 * (DV && DK ? 2 : 1) * DP / 32, COLUMN_READS, FINE ? 2 : MMAS>();
         }
     }
+    // (a key that does not count has P = 0, but 0 times an infinite or NaN grad_out is NaN)
+    if constexpr (DV) zero_unless(counts, dv);
+    if constexpr (DK) zero_unless(counts, dk);
     __syncthreads();                          // everybody is done with the tiles: their memory carries the results out
     constexpr int REGION = 2 * BUF / NW;
     char *region = lds + wave * REGION;

@@ -377,6 +377,14 @@ template <int N> __device__ __forceinline__ void clear(f32x16 (&a)[N])
         for (int r = 0; r < 16; ++r) a[i][r] = 0.f;
 }
 
+template <int N> __device__ __forceinline__ void zero_unless(bool keep, f32x16 (&a)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) a[i][r] = keep ? a[i][r] : 0.f;
+}
+
 // The result's 32 rows (lane = resident row, registers = head elements) times `f` to global memory, through LDS: a register holds 8 or
 // 16 bytes of 32 different rows, whole rows go out 16 bytes a lane.  `region`: BYTES of LDS of this wave; `dense`: the lane's own row
 // as an element offset from `out`, -1 for a row that is not there.  A wave writes and reads its own region only.

@@ -168,6 +168,7 @@ __global__ __launch_bounds__(2 * DP, 2) void short_kernel(cross_attention_args a
     int byte = 1;
     const auto word_of = [&](int t) -> uint32_t {
         if (!FEW_KEYS) return (uint32_t)__builtin_amdgcn_ballot_w64(byte == 0);
+        if (!keys) return 0;                   // (no key at all: no gradient, whatever grad_out holds)
         int g, first;
         place(t, g, first);
         const int n = a.Lq - first;
@@ -371,6 +372,10 @@ __global__ __launch_bounds__(2 * DP, 2) void short_kernel(cross_attention_args a
                 XATTN_SCHED_GROUP(0x8, M - STEPS);
             }
         }
+        if (!FEW_KEYS && word != ~0u) {        // (keys that do not count: 0 times an infinite or NaN grad_out is NaN)
+            zero_unless((word >> (lane & 31)) & 1, long1);
+            zero_unless((word >> (lane & 31)) & 1, long2);
+        }
         // (few keys: grad_query; few rows: grad_key, grad_value)
         MSDA_WAVE_LDS_SYNC();
 #pragma unroll
@@ -404,11 +409,13 @@ __global__ __launch_bounds__(2 * DP, 2) void short_kernel(cross_attention_args a
             dense = (((int64_t)b * a.Lq + q) * a.heads + hk * G + g) * a.D;
         }
         f32x16 v[1] = {sum1[i]};
+        if (FEW_KEYS) zero_unless((keys >> r) & 1, v);
         T *first = static_cast<T *>(FEW_KEYS ? a.grad_key : a.grad_query) + d0;
         if (splits == 1) put_rows<T, 32, OUT_REGION>(v, a.scale, mine, first, dense, a.D - d0, lane);
         else put_rows<float, 32, OUT_REGION>(v, 1.f, mine, partial, dense, a.D - d0, lane);
         if constexpr (FEW_KEYS) {
             v[0] = sum2[i];
+            zero_unless((keys >> r) & 1, v);
             if (splits == 1) put_rows<T, 32, OUT_REGION>(v, 1.f, mine, static_cast<T *>(a.grad_value) + d0, dense, a.D - d0, lane);
             else put_rows<float, 32, OUT_REGION>(v, 1.f, mine, partial + all, dense, a.D - d0, lane);
         }

@@ -19,3 +19,20 @@ def test_an_empty_axis_with_more_groups_than_the_card_holds(lib, Lq, Lk):  # noq
     x = make(1, Lq, Lk, 300, 300, 256, torch.float32)
     got = run(lib, x, 0.5)
     assert not any(bool(t.any()) for t in got.values())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("case", [(2, 70, 90, 2, 1, 32, False), (2, 70, 40, 2, 1, 128, False), (2, 20, 100, 2, 1, 128, False),
+                                  (2, 20, 100, 2, 2, 256, True)], ids=str)
+def test_masked_keys_get_zero_gradients_whatever_grad_out_holds(lib, case, dtype):  # noqa: F811
+    """a NaN and an infinite row of grad_out: P = 0 times them is NaN.  Keys that do not count, and queries without any key (the last
+    sequence), still get zeros; so do the keys that count in what the two rows do not reach"""
+    x = make(*case[:6], dtype, "hl", case[6], seed=4)
+    x["g"][:, 0], x["g"][:, 1] = float("nan"), float("inf")
+    got = run(lib, x, 0.2)
+    dead = x["dead"]
+    assert bool(dead[0].any()) and not bool(dead[0].all()) and bool(dead[-1].all())
+    for name in ("grad_key", "grad_value"):
+        assert not bool(got[name][dead].any()), name
+        assert bool(torch.isnan(got[name][~dead]).any()), name
+    assert not bool(got["grad_query"][-1].any()) and bool(torch.isfinite(got["grad_query"][0, 2:]).all())
