@@ -26,8 +26,8 @@ def cross_attention(query, key, value, key_padding_mask=None, key_lengths=None, 
     zero gradients; a query without any key gives zeros.
     scale: positive, 1 / sqrt(D) by default.  keep [B, H, Lq, Lk] bool or uint8: dropout mask of the probabilities, kept ones are
     multiplied by `keep_scale`.
-    Sums, maxima and gradients are accumulated in float32; calls are repeatable bit for bit.  Differentiable (once) in query,
-    key and value; capturable in a HIP graph."""
+    Sums, maxima and gradients are accumulated in float32; calls are repeatable bit for bit.  Differentiable (once, in
+    reverse mode) in query, key and value; capturable in a HIP graph."""
     for name, t in (("query", query), ("key", key), ("value", value)):
         if not isinstance(t, torch.Tensor) or t.dim() != 4:
             raise ValueError(f"cross_attention: {name} must be a [batch, tokens, heads, head size] tensor")

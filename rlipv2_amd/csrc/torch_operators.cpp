@@ -179,6 +179,9 @@ struct CrossAttentionFunction : public torch::autograd::Function<CrossAttentionF
 Tensor cross_attention(const Tensor &query, const Tensor &key, const Tensor &value, const Maybe &padding, const Maybe &lengths,
                        const Maybe &keep, double scale, double keep_scale)
 {
+    // (the kernels write through raw pointers: a tangent would be lost without a word)
+    for (const Tensor *t : {&query, &key, &value})
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "cross_attention: forward-mode derivatives are not implemented");
     if (at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad() || value.requires_grad()))
         return CrossAttentionFunction::apply(query, key, value, padding, lengths, keep, scale, keep_scale);
     return run_forward(query, key, value, padding, lengths, keep, scale, keep_scale, false).out;

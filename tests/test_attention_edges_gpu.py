@@ -48,3 +48,12 @@ def test_masked_keys_get_zero_gradients_whatever_grad_out_holds(case, dtype):
     for g in (gk, gv):
         assert not bool(g[dead].any()) and bool(torch.isnan(g[~dead]).any())
     assert not bool(gq[-1].any()) and bool(torch.isfinite(gq[0, 2:]).all())
+
+
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwad
+    x = [torch.randn(1, 3, 2, 8, device=DEV) for _ in range(3)]
+    with fwad.dual_level():
+        dual = fwad.make_dual(x[0], torch.ones_like(x[0]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            cross_attention(dual, x[1], x[2])
