@@ -40,20 +40,21 @@ void *stream_of(const at::Device &device) { return c10::hip::getCurrentHIPStream
 
 void check(int status, const char *name) { TORCH_CHECK(status == 0, name, ": ", entry.strerror(status)); }
 
-// The tensor itself where the kernels can read it: elements of a head contiguous, rows 16-byte aligned and less than 64 MB apart;
-// else a copy.
+// The tensor itself where the kernels can read it: elements of a head contiguous, rows 16-byte aligned and less than 64 MB apart (the
+// stride of a dimension of one element is never used: any value); else a copy.  A copy even of what counts as contiguous: contiguous()
+// would return the same memory.
 Tensor operand(const Tensor &t)
 {
     const int64_t unit = 16 / (int64_t)t.element_size();
-    const auto s = t.strides();
-    const bool fits = s[3] == 1 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0 && s[1] < ((int64_t)1 << 22) * unit &&
-                      reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
-    return fits ? t : t.contiguous();
+    bool fits = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i)
+        fits &= t.size(i) <= 1 || (t.stride(i) % unit == 0 && (i != 1 || t.stride(i) < ((int64_t)1 << 22) * unit));
+    return fits ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 void set_strides(int64_t (&to)[3], const Tensor &t)
 {
-    for (int i = 0; i < 3; ++i) to[i] = t.stride(i);
+    for (int i = 0; i < 3; ++i) to[i] = t.size(i) <= 1 ? 0 : t.stride(i);
 }
 
 const void *data(const Maybe &t) { return t && t->defined() ? t->const_data_ptr() : nullptr; }

@@ -57,3 +57,47 @@ def test_forward_mode_derivatives_are_refused():
         dual = fwad.make_dual(x[0], torch.ones_like(x[0]))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             cross_attention(dual, x[1], x[2])
+
+
+def at_odd_address(t):
+    """the same values as a contiguous view one element into a buffer"""
+    buf = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)
+    view = buf[1:].view(t.shape)
+    view.copy_(t)
+    assert view.is_contiguous() and view.data_ptr() % 16
+    return view
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("case", [(2, 5, 70, 2, 1, 32), (1, 1, 40, 2, 2, 128), (3, 20, 7, 1, 1, 8)], ids=str)
+def test_contiguous_operands_at_an_odd_address_are_copied(dtype, case):
+    x = make(*case, dtype, "h", seed=1, device=DEV)
+    want = run(x)
+    for names in (("q",), ("k",), ("v",), ("g",), ("q", "k", "v", "g")):
+        got = run(dict(x, **{n: at_odd_address(x[n]) for n in names}))
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), names
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_that_is_a_slice_of_a_concatenation(dtype):
+    """autograd hands over a contiguous view of the concatenation's gradient, behind an odd number of elements"""
+    x = make(1, 6, 9, 2, 2, 16, dtype, seed=2, device=DEV)
+    want = run(x)
+    q, k, v = (x[n].detach().requires_grad_(True) for n in ("q", "k", "v"))
+    other = torch.zeros(3, dtype=dtype, device=DEV, requires_grad=True)
+    both = torch.cat((other, cross_attention(q, k, v).flatten()))
+    got = torch.autograd.grad(both, (q, k, v), torch.cat((torch.ones(3, dtype=dtype, device=DEV), x["g"].flatten())))
+    assert all(torch.equal(a, b) for a, b in zip(got, want[1:]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_strides_of_dimensions_of_one_element_are_ignored(dtype):
+    """one sequence cut out of rows with a pad, one token and one head out of odd buffers: such strides are arbitrary"""
+    x = make(1, 1, 50, 1, 1, 64, dtype, "h", seed=3, device=DEV)
+    want = run(x)
+    odd = lambda t, i: t.as_strided(t.shape, tuple(s if j != i else 12803 for j, s in enumerate(t.stride())))
+    far = lambda t: t.as_strided(t.shape, tuple(s if j != 1 else 1 << 40 for j, s in enumerate(t.stride())))
+    for change in ({"q": odd(x["q"], 0)}, {"q": odd(x["q"], 1)}, {"q": odd(x["q"], 2)}, {"k": odd(x["k"], 0), "v": odd(x["v"], 2)},
+                   {"g": odd(x["g"], 1)}, {"q": far(x["q"]), "g": far(x["g"])}):
+        got = run(dict(x, **change))
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), change.keys()
