@@ -462,7 +462,7 @@ size_t backward_workspace(const cross_attention_args &a)
 {
     if (const int side = short_side(a)) {
         const int splits = short_splits(a);
-        return splits == 1 ? 0 : (size_t)splits * (side == 1 ? 2 * (size_t)a.Lk * a.kv_heads : (size_t)a.Lq * a.heads) * a.B * a.D * sizeof(float);
+        return splits == 1 || !a.grad_key ? 0 : (size_t)splits * (side == 1 ? 2 * (size_t)a.Lk * a.kv_heads : (size_t)a.Lq * a.heads) * a.B * a.D * sizeof(float);
     }
     const Plan pq = query_plan(a), pk = a.grad_key ? key_plan(a) : Plan{1, 1, 1};
     const size_t q = pq.splits == 1 ? 0 : (size_t)pq.splits * a.B * a.Lq * a.heads * a.D * sizeof(float);
@@ -475,9 +475,9 @@ int backward(const cross_attention_args &a, hipStream_t stream)
     if (const int side = short_side(a)) {
         const int splits = short_splits(a);
         launch_short(a, splits, stream);
-        if (splits > 1 && side == 1)
+        if (splits > 1 && side == 1 && a.grad_key)
             reduce<bf16_t>(a, splits, (int64_t)a.B * a.Lk * a.kv_heads * a.D, a.scale, a.grad_key, 1.f, a.grad_value, stream);
-        else if (splits > 1)
+        else if (splits > 1 && side == 2)
             reduce<bf16_t>(a, splits, (int64_t)a.B * a.Lq * a.heads * a.D, a.scale, a.grad_query, 0.f, nullptr, stream);
         return hipGetLastError() == hipSuccess ? MSDA_OK : MSDA_ERR_LAUNCH;
     }
@@ -543,7 +543,7 @@ extern "C" int cross_attention_supported(const cross_attention_args *a)
     return a && (a->dtype == MSDA_BF16 || a->dtype == MSDA_F32) && xattn::sizes_ok(*a) && a->scale > 0.f && a->scale < kInf;
 }
 
-extern "C" int cross_attention_short_keys(const cross_attention_args *a) { return a && a->dtype == MSDA_BF16 && a->D > 64 && a->Lk <= 64; }
+extern "C" int cross_attention_short_keys(const cross_attention_args *a) { return cross_attention_supported(a) && xattn::short_side(*a) == 1; }
 
 extern "C" size_t cross_attention_workspace_bytes(const cross_attention_args *a, int backward)
 {

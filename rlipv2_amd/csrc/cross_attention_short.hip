@@ -391,6 +391,7 @@ __global__ __launch_bounds__(2 * DP, 2) void short_kernel(cross_attention_args a
         MSDA_WAVE_LDS_SYNC();
     }
     if (t0 < t1) leave(t1 - 1);
+    if (FEW_KEYS && !a.grad_key) return;
     __syncthreads();                           // everybody is done with the tiles: their memory carries the short gradients out
 
     constexpr int OUT_REGION = 2 * BUF / WAVES;
@@ -422,11 +423,12 @@ __global__ __launch_bounds__(2 * DP, 2) void short_kernel(cross_attention_args a
     }
 }
 
-// Which of the two kernels a call takes: 1 few keys, 2 few rows, 0 neither.
+// Which of the two kernels a call takes: 1 few keys (also for the query's gradient alone: the forward call, which does not know what will
+// be asked for, leaves out out_low), 2 few rows, 0 neither.
 int short_side(const cross_attention_args &a)
 {
-    if (a.dtype != MSDA_BF16 || a.D <= 64 || !a.grad_key || a.Lq == 0 || a.Lk == 0 || a.heads > (1 << 16)) return 0;
-    return a.Lk <= 64 ? 1 : (int64_t)(a.heads / a.kv_heads) * a.Lq <= 64 ? 2 : 0;
+    if (a.dtype != MSDA_BF16 || a.D <= 64 || a.Lq == 0 || a.Lk == 0 || a.heads > (1 << 16)) return 0;
+    return a.Lk <= 64 ? 1 : a.grad_key && (int64_t)(a.heads / a.kv_heads) * a.Lq <= 64 ? 2 : 0;
 }
 
 int short_splits(const cross_attention_args &a)

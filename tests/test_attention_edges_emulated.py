@@ -7,6 +7,7 @@ import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "tests"))
+from attention_delta import CASES, check_grad_query, inputs  # noqa: E402
 from attention_reference import make  # noqa: E402
 from test_attention_emulated import CLANG, lib, run  # noqa: E402, F401
 
@@ -36,3 +37,11 @@ def test_masked_keys_get_zero_gradients_whatever_grad_out_holds(lib, case, dtype
         assert not bool(got[name][dead].any()), name
         assert bool(torch.isnan(got[name][~dead]).any()), name
     assert not bool(got["grad_query"][-1].any()) and bool(torch.isfinite(got["grad_query"][0, 2:]).all())
+
+
+@pytest.mark.parametrize("states", [True, False])
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_delta_does_not_carry_the_rounding_of_the_result(lib, case, states):  # noqa: F811
+    """also where only the query is trained"""
+    x = inputs(case)
+    check_grad_query(run(lib, x, 0.3, states)["grad_query"], x, 0.3)

@@ -7,6 +7,7 @@ import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "tests"))
+from attention_delta import CASES, check_grad_query, inputs  # noqa: E402
 from attention_reference import make  # noqa: E402
 
 from rlipv2_amd.attention import cross_attention  # noqa: E402
@@ -101,3 +102,12 @@ def test_strides_of_dimensions_of_one_element_are_ignored(dtype):
                    {"g": odd(x["g"], 1)}, {"q": far(x["q"]), "g": far(x["g"])}):
         got = run(dict(x, **change))
         assert all(torch.equal(a, b) for a, b in zip(got, want)), change.keys()
+
+
+@pytest.mark.parametrize("states", ["trained", "frozen", "asked for the query alone"])
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_delta_does_not_carry_the_rounding_of_the_result(case, states):
+    x = inputs(case, DEV)
+    q, k, v = (x[n].detach().requires_grad_(n == "q" or states != "frozen") for n in ("q", "k", "v"))
+    out = cross_attention(q, k, v, scale=0.3)
+    check_grad_query(torch.autograd.grad(out, (q, k, v) if states == "trained" else (q,), x["g"])[0], x, 0.3)
