@@ -50,7 +50,8 @@ typedef struct cross_attention_args {
     int64_t grad_out_stride[3];
     void *grad_query, *grad_key, *grad_value;
     void *delta;
-    /* cross_attention_workspace_bytes(args, backward) bytes of device memory, 16-byte aligned (may be NULL if that is 0) */
+    /* cross_attention_workspace_bytes(args, backward) bytes of device memory, 16-byte aligned (may be NULL if that is 0): partial results
+     * of as many workgroups as fit on the card, and for long float32 forward calls 8 bytes a query row */
     void *workspace;
     size_t workspace_bytes;
 } cross_attention_args;

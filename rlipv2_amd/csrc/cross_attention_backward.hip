@@ -24,7 +24,7 @@ using namespace xattn;
 
 // KEEP: with a dropout mask
 template <typename T, int DP, int NW, int BN, int OCC, bool KEEP, bool FINE>
-__global__ __launch_bounds__(64 * NW, OCC) void query_kernel(cross_attention_args a, int row_tiles, int splits, float c)
+__global__ __launch_bounds__(64 * NW, OCC) void query_kernel(cross_attention_args a, int row_tiles, int splits, Stretch stretch, float c)
 {
     constexpr int THREADS = 64 * NW, NSUB = BN / 32, KB = BN * Tile<T, DP>::ROW, BUF = 2 * KB;
     constexpr bool AHEAD = sizeof(T) == 2 && !KEEP;      // (float32: eight matrix instructions per operand; the schedule takes minutes to compile)
@@ -83,7 +83,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void query_kernel(cross_attention_arg
     KeyMask mask;
     mask.init(a, b);
     const int tiles = (mask.length + BN - 1) / BN, per = (tiles + splits - 1) / splits;
-    const int t0 = min(sp * per, tiles), t1 = min(tiles, t0 + per);
+    int t0 = min(sp * per, tiles), t1 = min(tiles, t0 + per);
+    take_stretch<T, BN>(stretch, t0, t1);
     const int my_key = lane & (BN - 1);
     Stager<T, DP, BN, THREADS> kstage, vstage;
     kstage.init(a.key_stride[1], tid, a.D);
@@ -162,17 +163,19 @@ __global__ __launch_bounds__(64 * NW, OCC) void query_kernel(cross_attention_arg
             ahead<AHEAD, 2 * DP / 32, COLUMN_READS, FINE ? 2 : MMAS>();
         }
     }
+    float *part = static_cast<float *>(a.workspace) + (int64_t)sp * a.B * a.Lq * a.heads * a.D;
+    if (sizeof(T) == 4 && stretch.index > 0 && ok) add_row(acc, (splits == 1 ? static_cast<const float *>(a.grad_query) : part) + dense, 1.f, a.D, half);
+    const float factor = sizeof(T) == 4 && stretch.index + 1 < stretch.count ? 1.f : a.scale;
     __syncthreads();                          // everybody is done with the tiles: their memory carries the results out
     constexpr int REGION = 2 * BUF / NW;
     char *region = lds + wave * REGION;
-    if (splits == 1) put_rows<T, DP, REGION>(acc, a.scale, region, static_cast<T *>(a.grad_query), ok ? dense : -1, a.D, lane);
-    else put_rows<float, DP, REGION>(acc, 1.f, region, static_cast<float *>(a.workspace) + (int64_t)sp * a.B * a.Lq * a.heads * a.D,
-                                     ok ? dense : -1, a.D, lane);
+    if (splits == 1) put_rows<T, DP, REGION>(acc, factor, region, static_cast<T *>(a.grad_query), ok ? dense : -1, a.D, lane);
+    else put_rows<float, DP, REGION>(acc, 1.f, region, part, ok ? dense : -1, a.D, lane);
 }
 
 // DV / DK: which of the two gradients this launch computes (float32 heads of 256: one at a time, the registers do not hold both)
 template <typename T, int DP, int NW, int BM, int OCC, bool DV, bool DK, bool KEEP, bool FINE>
-__global__ __launch_bounds__(64 * NW, OCC) void key_kernel(cross_attention_args a, int key_tiles, int splits, float c)
+__global__ __launch_bounds__(64 * NW, OCC) void key_kernel(cross_attention_args a, int key_tiles, int splits, Stretch stretch, float c)
 {
     constexpr int THREADS = 64 * NW, NSUB = BM / 32, QB = BM * Tile<T, DP>::ROW, BUF = 2 * QB;
     constexpr bool AHEAD = sizeof(T) == 2 && !KEEP;      // (float32: eight matrix instructions per operand; the schedule takes minutes to compile)
@@ -206,7 +209,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void key_kernel(cross_attention_args 
     }
     // a tile of rows belongs to one query head: tile t is head g = t / head_tiles of those that share the key head
     const int head_tiles = (a.Lq + BM - 1) / BM, tiles = G * head_tiles, per = (tiles + splits - 1) / splits;
-    const int t0 = min(sp * per, tiles), t1 = __builtin_amdgcn_ballot_w64(counts) || NW > 1 ? min(tiles, t0 + per) : t0;
+    int t0 = min(sp * per, tiles), t1 = __builtin_amdgcn_ballot_w64(counts) || NW > 1 ? min(tiles, t0 + per) : t0;
+    take_stretch<T, BM>(stretch, t0, t1);
     Stager<T, DP, BM, THREADS> qstage, gstage;
     qstage.init(a.query_stride[1], tid, a.D);
     gstage.init(a.grad_out_stride[1], tid, a.D);
@@ -327,20 +331,25 @@ __global__ __launch_bounds__(64 * NW, OCC) void key_kernel(cross_attention_args 
             ahead<AHEAD, 2 * (DV && DK ? 2 : 1) * DP / 32, COLUMN_READS, FINE ? 2 : MMAS>();
         }
     }
+    const int64_t dense = key < a.Lk ? (((int64_t)b * a.Lk + key) * a.kv_heads + hk) * a.D : -1, all = (int64_t)a.B * a.Lk * a.kv_heads * a.D;
+    float *part = static_cast<float *>(a.workspace) + (int64_t)sp * 2 * all;
+    if (sizeof(T) == 4 && stretch.index > 0 && dense >= 0) {
+        if constexpr (DV) add_row(dv, (splits == 1 ? static_cast<const float *>(a.grad_value) : part) + dense, 1.f, a.D, half);
+        if constexpr (DK) add_row(dk, (splits == 1 ? static_cast<const float *>(a.grad_key) : part + all) + dense, 1.f, a.D, half);
+    }
+    const float factor = sizeof(T) == 4 && stretch.index + 1 < stretch.count ? 1.f : a.scale;
     // (a key that does not count has P = 0, but 0 times an infinite or NaN grad_out is NaN)
     if constexpr (DV) zero_unless(counts, dv);
     if constexpr (DK) zero_unless(counts, dk);
     __syncthreads();                          // everybody is done with the tiles: their memory carries the results out
     constexpr int REGION = 2 * BUF / NW;
     char *region = lds + wave * REGION;
-    const int64_t dense = key < a.Lk ? (((int64_t)b * a.Lk + key) * a.kv_heads + hk) * a.D : -1, all = (int64_t)a.B * a.Lk * a.kv_heads * a.D;
-    float *part = static_cast<float *>(a.workspace) + (int64_t)sp * 2 * all;
     if constexpr (DV) {
         if (splits == 1) put_rows<T, DP, REGION>(dv, 1.f, region, static_cast<T *>(a.grad_value), dense, a.D, lane);
         else put_rows<float, DP, REGION>(dv, 1.f, region, part, dense, a.D, lane);
     }
     if constexpr (DK) {
-        if (splits == 1) put_rows<T, DP, REGION>(dk, a.scale, region, static_cast<T *>(a.grad_key), dense, a.D, lane);
+        if (splits == 1) put_rows<T, DP, REGION>(dk, factor, region, static_cast<T *>(a.grad_key), dense, a.D, lane);
         else put_rows<float, DP, REGION>(dk, 1.f, region, part + all, dense, a.D, lane);
     }
 }
@@ -374,13 +383,13 @@ Plan query_plan(const cross_attention_args &a)
 {
     const int bytes = row_bytes(a), n = rows_per_tile(bytes);
     return plan_for((int64_t)(a.heads / a.kv_heads) * a.Lq, (a.Lk + n - 1) / n, (int64_t)a.B * a.kv_heads, tile_lds(a),
-                    bytes <= 64 ? 4 : bytes <= 128 ? 3 : bytes <= 256 ? 2 : 1, least_tiles(a), most_tiles(a));
+                    bytes <= 64 ? 4 : bytes <= 128 ? 3 : bytes <= 256 ? 2 : 1, least_tiles(a));
 }
 Plan key_plan(const cross_attention_args &a)
 {
     const int bytes = row_bytes(a), n = rows_per_tile(bytes);
     return plan_for(a.Lk, (int64_t)(a.heads / a.kv_heads) * ((a.Lq + n - 1) / n), (int64_t)a.B * a.kv_heads, tile_lds(a),
-                    bytes <= 64 ? 3 : bytes <= 256 ? 2 : 1, least_tiles(a), most_tiles(a));
+                    bytes <= 64 ? 3 : bytes <= 256 ? 2 : 1, least_tiles(a));
 }
 
 template <typename T, int DP, int NW, bool KEEP, bool FINE> void launch_query(const cross_attention_args &a, const Plan &p, float c, hipStream_t stream)
@@ -388,8 +397,10 @@ template <typename T, int DP, int NW, bool KEEP, bool FINE> void launch_query(co
     constexpr int BN = rows_per_tile(Tile<T, DP>::ROW), LDS = 4 * BN * Tile<T, DP>::ROW + 2 * BN * 4, OCC = DP * (int)sizeof(T) >= 512 ? 1 : 2;
     const auto kernel = query_kernel<T, DP, NW, BN, OCC, KEEP, FINE>;
     RLIPV2_ONCE_PER_DEVICE((void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)p.tiles * p.splits * a.B * a.kv_heads)), dim3(64 * NW), LDS, stream, a, p.tiles,
-                       p.splits, c);
+    const int stretches = stretches_of(a, (a.Lk + BN - 1) / BN, p);
+    for (int i = 0; i < stretches; ++i)
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)p.tiles * p.splits * a.B * a.kv_heads)), dim3(64 * NW), LDS, stream, a, p.tiles,
+                           p.splits, Stretch{i, stretches}, c);
     if (p.splits > 1) {
         const int64_t n = (int64_t)a.B * a.Lq * a.heads * a.D;
         reduce<T>(a, p.splits, n, a.scale, a.grad_query, 0.f, nullptr, stream);
@@ -401,8 +412,10 @@ template <typename T, int DP, int NW, bool DV, bool DK, bool KEEP, bool FINE> vo
     constexpr int BM = rows_per_tile(Tile<T, DP>::ROW), LDS = 4 * BM * Tile<T, DP>::ROW + 4 * BM * 4, OCC = DP * (int)sizeof(T) >= 512 ? 1 : 2;
     const auto kernel = key_kernel<T, DP, NW, BM, OCC, DV, DK, KEEP, FINE>;
     RLIPV2_ONCE_PER_DEVICE((void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)p.tiles * p.splits * a.B * a.kv_heads)), dim3(64 * NW), LDS, stream, a, p.tiles,
-                       p.splits, c);
+    const int stretches = stretches_of(a, (int64_t)(a.heads / a.kv_heads) * ((a.Lq + BM - 1) / BM), p);
+    for (int i = 0; i < stretches; ++i)
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)p.tiles * p.splits * a.B * a.kv_heads)), dim3(64 * NW), LDS, stream, a, p.tiles,
+                           p.splits, Stretch{i, stretches}, c);
 }
 
 template <typename T, int DP, int NW, bool KEEP, bool FINE> void launch_key(const cross_attention_args &a, const Plan &p, float c, hipStream_t stream)

@@ -432,14 +432,48 @@ __device__ __forceinline__ void put_rows(const f32x16 (&acc)[DP / 32], float f, 
     }
 }
 
+// A float32 accumulator takes at most 2048 streamed rows in sequence, because its rounding error grows with their number.  A split with
+// more is cut into stretches, a launch each (2048 rows of a full card are long enough for one): all but the last leave their float32 sums,
+// not scaled, where the result or the split's partial result goes, and a launch adds what the one before left.  Memory for the
+// stretches themselves would grow with the product of the lengths; adding up inside the loop cost the registers of the heads of 256 (5000
+// rows over 5000 keys, 16 heads: 23 -> 36 ms).
+constexpr int kStretch = 2048;
+struct Stretch { int index, count; };
+
+// tiles [t0, t1) of this stretch of a split's
+template <typename T, int ROWS> __device__ __forceinline__ void take_stretch(const Stretch &s, int &t0, int &t1)
+{
+    if (sizeof(T) == 2) return;
+    t0 = min(t0 + s.index * (kStretch / ROWS), t1);
+    t1 = min(t0 + kStretch / ROWS, t1);
+}
+
+// acc += f times this lane's row (lane & 31) in memory
+template <int N> __device__ __forceinline__ void add_row(f32x16 (&acc)[N], const float *row, float f, int D, int half)
+{
+#pragma unroll
+    for (int dt = 0; dt < N; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = dt * 32 + 8 * g + 4 * half;
+            if (d < D) {
+                const float4 v = *reinterpret_cast<const float4 *>(row + d);
+                acc[dt][4 * g] = fmaf(v.x, f, acc[dt][4 * g]);
+                acc[dt][4 * g + 1] = fmaf(v.y, f, acc[dt][4 * g + 1]);
+                acc[dt][4 * g + 2] = fmaf(v.z, f, acc[dt][4 * g + 2]);
+                acc[dt][4 * g + 3] = fmaf(v.w, f, acc[dt][4 * g + 3]);
+            }
+        }
+}
+
 // ---- host: how a call is cut --------------------------------------------------------------------------------------------------
 struct Plan { int waves, tiles, splits; };
 
 // `resident` rows of each of `groups` (batch, key head) pairs are held 32 per wave, one, two or four waves a workgroup.  Where that does
 // not fill the card the streamed tiles are cut into splits: as many as all fit on the 256 compute units at once, by LDS and by the
-// waves a SIMD holds, with at least `least` and at most `longest` tiles each.  Measured (bf16): twice as many cost the partial results' traffic -- 64 rows of
+// waves a SIMD holds, with at least `least` tiles each.  Measured (bf16): twice as many cost the partial results' traffic -- 64 rows of
 // heads of 256 over 22 223 keys 147 us with one round, 163 with two, 193 with four; four shared heads of 128 129 / 134 / 145 us.
-inline Plan plan_for(int64_t resident, int64_t streamed_tiles, int64_t groups, int lds, int waves_per_simd, int least, int longest)
+inline Plan plan_for(int64_t resident, int64_t streamed_tiles, int64_t groups, int lds, int waves_per_simd, int least)
 {
     Plan p;
     int64_t most = streamed_tiles / least > 1 ? streamed_tiles / least : 1;
@@ -450,9 +484,8 @@ inline Plan plan_for(int64_t resident, int64_t streamed_tiles, int64_t groups, i
     // (half of the compute units have work already: joining pays from 16 tiles a split on -- 2331 rows of heads of 64 over 1091 keys
     // 24.6 us with one split, 30.5 with three)
     if (have >= 128 && least == 4) most = streamed_tiles / 16 > 1 ? streamed_tiles / 16 : 1;
-    const int64_t split = have ? 256 * (int64_t)fit / have : 1, fewest = streamed_tiles > longest ? (streamed_tiles + longest - 1) / longest : 1;
-    if (most < fewest) most = fewest;
-    p.splits = (int)(split < fewest ? fewest : split > most ? most : split);        // (one where nothing is streamed)
+    const int64_t split = have ? 256 * (int64_t)fit / have : 1;
+    p.splits = (int)(split < 1 ? 1 : split > most ? most : split);
     return p;
 }
 
@@ -473,7 +506,11 @@ inline bool few_probabilities(const cross_attention_args &a)
     return a.dtype == MSDA_BF16 && !a.keep && (double)a.B * a.heads * a.Lq * a.Lk <= 1 << 24;
 }
 
-// a float32 accumulator takes at most 2048 streamed rows in sequence: its rounding error grows with their number
-inline int most_tiles(const cross_attention_args &a) { return a.dtype == MSDA_BF16 ? 1 << 30 : 2048 / rows_per_tile(row_bytes(a)); }
+// stretches (add_row) of a split of `tiles` tiles
+inline int stretches_of(const cross_attention_args &a, int64_t tiles, const Plan &p)
+{
+    const int64_t per = (tiles + p.splits - 1) / p.splits, most = kStretch / rows_per_tile(row_bytes(a));
+    return a.dtype == MSDA_BF16 || per <= most ? 1 : (int)((per + most - 1) / most);
+}
 
 }  // namespace xattn

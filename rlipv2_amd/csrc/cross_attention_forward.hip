@@ -30,7 +30,7 @@ using namespace xattn;
 
 // KEEP: with a dropout mask
 template <typename T, int DP, int NW, int BN, int OCC, bool KEEP>
-__global__ __launch_bounds__(64 * NW, OCC) void forward_kernel(cross_attention_args a, int row_tiles, int splits, float c)
+__global__ __launch_bounds__(64 * NW, OCC) void forward_kernel(cross_attention_args a, int row_tiles, int splits, Stretch stretch, float c)
 {
     constexpr int THREADS = 64 * NW, NSUB = BN / 32, KB = BN * Tile<T, DP>::ROW, BUF = 2 * KB;
     constexpr bool AHEAD = !KEEP;
@@ -64,7 +64,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void forward_kernel(cross_attention_a
     KeyMask mask;
     mask.init(a, b);
     const int tiles = (mask.length + BN - 1) / BN, per = (tiles + splits - 1) / splits;
-    const int t0 = min(sp * per, tiles), t1 = min(tiles, t0 + per);
+    int t0 = min(sp * per, tiles), t1 = min(tiles, t0 + per);
+    take_stretch<T, BN>(stretch, t0, t1);
     const int my_key = lane & (BN - 1);
     Stager<T, DP, BN, THREADS> kstage, vstage;
     kstage.init(a.key_stride[1], tid, a.D);
@@ -78,7 +79,15 @@ __global__ __launch_bounds__(64 * NW, OCC) void forward_kernel(cross_attention_a
 
     f32x16 acc[DP / 32];
     clear(acc);
+    const int64_t at = ((int64_t)sp * a.B * a.kv_heads + bh) * rows.count + r, all = (int64_t)splits * a.B * a.kv_heads * rows.count;
+    float *part = static_cast<float *>(a.workspace), *held = part + (splits == 1 ? 0 : all * (a.D + 1)) + 2 * at;
     float m = -kInf, scaled = -kInf, l = 0.f; // the maximum, c times it as the exponents subtract it; l: this half's keys only
+    // (float32: held = the maximum and the sum that the stretches before left; the sum's halves meet at the end)
+    const bool more = sizeof(T) == 4 && stretch.index > 0 && ok;
+    if (more) {
+        m = held[0];
+        scaled = m * c;
+    }
     unsigned long long word = 0, next = 0;
     int byte = 1;
     constexpr unsigned long long ALL = BN == 64 ? ~0ull : 0xffffffffull;
@@ -166,23 +175,35 @@ __global__ __launch_bounds__(64 * NW, OCC) void forward_kernel(cross_attention_a
         ahead<AHEAD, NSUB * 2 * DP / 32, COLUMN_READS, MMAS>();
     }
 
+    const int64_t dense = (((int64_t)b * a.Lq + q) * a.heads + head) * a.D;
+    if (more) {
+        const float f = exp2_fast(held[0] * c - (scaled == -kInf ? 0.f : scaled));
+        add_row(acc, splits == 1 ? static_cast<const float *>(a.out) + dense : part + at * a.D, f, a.D, half);
+        if (half == 0) l = fmaf(held[1], f, l);
+    }
     const float total = l + other_half(l);
     const float inv = total == 0.f ? 0.f : 1.f / total, log_sum = scaled + log2_fast(total);
     __syncthreads();                          // everybody is done with the tiles: their memory carries the results out
     constexpr int REGION = 2 * BUF / NW;
     char *region = lds + wave * REGION;
+    if (sizeof(T) == 4 && stretch.index + 1 < stretch.count) {
+        float *to = splits == 1 ? static_cast<float *>(a.out) : part;
+        put_rows<float, DP, REGION>(acc, 1.f, region, to, !ok ? -1 : splits == 1 ? dense : at * a.D, a.D, lane);
+        if (ok && half == 0) {
+            held[0] = m;
+            held[1] = total;
+        }
+        return;
+    }
     if (splits == 1) {
-        const int64_t dense = (((int64_t)b * a.Lq + q) * a.heads + head) * a.D;
         put_rows<T, DP, REGION>(acc, inv, region, static_cast<T *>(a.out), ok ? dense : -1, a.D, lane);
         if (sizeof(T) == 2 && a.out_low)
             put_rows<T, DP, REGION, true>(acc, inv, region, static_cast<T *>(a.out_low), ok ? dense : -1, a.D, lane);
         if (a.stats && ok && half == 0)
             static_cast<float *>(a.stats)[((int64_t)b * a.heads + head) * a.Lq + q] = total == 0.f ? kInf : log_sum;
     } else {
-        const int64_t at = ((int64_t)sp * a.B * a.kv_heads + bh) * rows.count + r;
-        float *part = static_cast<float *>(a.workspace);
         put_rows<float, DP, REGION>(acc, inv, region, part, ok ? at * a.D : -1, a.D, lane);
-        if (ok && half == 0) part[(int64_t)splits * a.B * a.kv_heads * rows.count * a.D + at] = total == 0.f ? -kInf : log_sum;
+        if (ok && half == 0) part[all * a.D + at] = total == 0.f ? -kInf : log_sum;
     }
 }
 
@@ -243,7 +264,7 @@ Plan plan_of(const cross_attention_args &a)
 {
     const int bytes = row_bytes(a), n = rows_per_tile(bytes);
     return plan_for((int64_t)(a.heads / a.kv_heads) * a.Lq, (a.Lk + n - 1) / n, (int64_t)a.B * a.kv_heads, tile_lds(a),
-                    bytes <= 64 ? 4 : bytes <= 128 ? 3 : bytes <= 512 ? 2 : 1, least_tiles(a), most_tiles(a));
+                    bytes <= 64 ? 4 : bytes <= 128 ? 3 : bytes <= 512 ? 2 : 1, least_tiles(a));
 }
 
 template <typename T, int DP, int NW, bool KEEP> int launch(const cross_attention_args &a, const Plan &p, hipStream_t stream)
@@ -252,8 +273,10 @@ template <typename T, int DP, int NW, bool KEEP> int launch(const cross_attentio
     const auto kernel = forward_kernel<T, DP, NW, BN, OCC, KEEP>;
     RLIPV2_ONCE_PER_DEVICE((void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
     const int64_t groups = (int64_t)p.tiles * p.splits * a.B * a.kv_heads;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(64 * NW), LDS, stream, a, p.tiles, p.splits,
-                       a.scale * 1.4426950408889634f);
+    const int stretches = stretches_of(a, (a.Lk + BN - 1) / BN, p);
+    for (int i = 0; i < stretches; ++i)
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(64 * NW), LDS, stream, a, p.tiles, p.splits, Stretch{i, stretches},
+                           a.scale * 1.4426950408889634f);
     if (p.splits > 1) {
         int Q = 2, G = 1;
         while (Q < a.D / 4) Q *= 2;
@@ -287,7 +310,9 @@ namespace xattn {
 size_t forward_workspace(const cross_attention_args &a)
 {
     const Plan p = plan_of(a);
-    return p.splits == 1 ? 0 : (size_t)p.splits * a.B * a.heads * a.Lq * (a.D + 1) * sizeof(float);
+    const int n = rows_per_tile(row_bytes(a));
+    const size_t rows = (size_t)p.splits * a.B * a.heads * a.Lq, held = stretches_of(a, (a.Lk + n - 1) / n, p) > 1 ? 2 : 0;
+    return rows * ((p.splits == 1 ? 0 : a.D + 1) + held) * sizeof(float);
 }
 
 int forward(const cross_attention_args &a, hipStream_t stream)

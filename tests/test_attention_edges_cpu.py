@@ -1,9 +1,15 @@
 """Cross attention: what its host side refuses before any kernel."""
+import os
+import sys
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
 
 from rlipv2_amd import _lib
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from attention_reference import BACK, HEAD, NO_WORK  # noqa: E402
 
 
 @pytest.mark.parametrize("which", [0, 1, 2])
@@ -17,3 +23,16 @@ def test_forward_mode_derivatives_are_refused(which, requires_grad):
             x[(which + 1) % 3].requires_grad_(True)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             _lib.operators().cross_attention(*x, None, None, None, 0.3, 1.0)
+
+
+@pytest.mark.parametrize("B,Lq,Lk,H,Hk,D", [(4, 22223, 22223, 8, 8, 256), (1, 65536, 65536, 32, 8, 128), (1, 300, 22223, 64, 64, 256),
+                                            (1, 1, 1 << 24, 8, 8, 128), (1, 1 << 24, 64, 8, 8, 256), (16, 1 << 20, 1 << 20, 16, 16, 32)])
+@pytest.mark.parametrize("dtype", [_lib.MSDA_F32, _lib.MSDA_BF16])
+def test_workspaces_do_not_grow_with_the_product_of_the_lengths(dtype, B, Lq, Lk, H, Hk, D):
+    """splits only fill the card: at most as many workgroups as fit on it, each with 128 rows of two float32 results of 256 elements; a
+    float32 row of several stretches keeps its maximum and its sum"""
+    L = _lib.lib()
+    for backward in (0, 1):
+        head = HEAD.pack(dtype, B, H, Hk, Lq, Lk, D, 1.0, 1.0, 0, 16, 16, 16, *(0,) * 9, 0, 0, 0, 0, 16, 0, 16)
+        need = L.cross_attention_workspace_bytes(head + BACK.pack(16, 0, 0, 0, 16, 16, 16, 16) + NO_WORK, backward)
+        assert need <= 256 * 9 * 128 * 2 * 256 * 4 + B * H * Lq * 8, need

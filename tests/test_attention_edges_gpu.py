@@ -8,7 +8,7 @@ import torch
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "tests"))
 from attention_delta import CASES, check_grad_query, inputs  # noqa: E402
-from attention_reference import make  # noqa: E402
+from attention_reference import check, make, reference  # noqa: E402
 
 from rlipv2_amd.attention import cross_attention  # noqa: E402
 
@@ -111,3 +111,29 @@ def test_delta_does_not_carry_the_rounding_of_the_result(case, states):
     q, k, v = (x[n].detach().requires_grad_(n == "q" or states != "frozen") for n in ("q", "k", "v"))
     out = cross_attention(q, k, v, scale=0.3)
     check_grad_query(torch.autograd.grad(out, (q, k, v) if states == "trained" else (q,), x["g"])[0], x, 0.3)
+
+
+@pytest.mark.parametrize("case", [(1, 3, 5000, 260, 260, 128, "h"), (1, 5000, 3, 260, 260, 128, ""), (1, 2, 4200, 300, 300, 256, "hl"),
+                                  (1, 4200, 2, 300, 300, 256, "f"), (2, 5, 9000, 600, 300, 32, "hl"), (1, 2, 9000, 150, 150, 128, "h"),
+                                  (1, 4500, 33, 70, 70, 200, "h")], ids=str)
+def test_float32_sums_of_several_stretches(case):
+    """a card full of groups leaves one or two splits, whose float32 sums are added up in memory every 2048 rows"""
+    x = make(*case[:6], torch.float32, case[6], seed=sum(case[:6]), device=DEV)
+    names = ("out", "grad_query", "grad_key", "grad_value")
+    got = dict(zip(names, run(x, 0.1)))
+    check(got, reference(x["q"], x["k"], x["v"], x["g"], x["dead"], 0.1))
+    again = dict(zip(names, run(x, 0.1)))
+    assert all(torch.equal(got[n], again[n]) for n in names)
+
+
+def test_float32_rows_whose_maximum_grows_from_stretch_to_stretch():
+    """the logits rise along the keys, so that every stretch scales down what was held; masked stretches in front, between and behind"""
+    B, Lq, Lk, H, D = 1, 2, 9000, 260, 128
+    x = make(B, Lq, Lk, H, H, D, torch.float32, seed=9, device=DEV)
+    x["q"].fill_(1.0)
+    x["k"].mul_(0.01).add_(torch.linspace(-2.0, 2.0, Lk, device=DEV)[None, :, None, None])
+    x["padding"] = torch.zeros(B, Lk, dtype=torch.bool, device=DEV)
+    x["padding"][:, :2500] = x["padding"][:, 4000:6300] = x["padding"][:, 8200:] = True
+    x["dead"] = x["padding"]
+    got = dict(zip(("out", "grad_query", "grad_key", "grad_value"), run(x, 0.25)))
+    check(got, reference(x["q"], x["k"], x["v"], x["g"], x["dead"], 0.25))
