@@ -501,13 +501,11 @@ bool sizes_ok(const cross_attention_args &a)
 {
     if (a.B < 0 || a.Lq < 0 || a.Lk < 0 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads) return false;
     if (a.D < 8 || a.D > 256 || a.D % 8) return false;
-    // rows of a key head and workgroups of a launch are counted in 32 bits (a split side is at most 2048 workgroups more)
-    const int64_t limit = (int64_t)1 << 30, rows = (int64_t)(a.heads / a.kv_heads) * a.Lq;
-    if (rows > limit || a.Lk > limit) return false;
-    const int64_t groups = ((rows > a.Lk ? rows : a.Lk) / 32 + 1);
-    if ((int64_t)a.B * a.kv_heads > limit / groups) return false;
-    // the joining kernels count four elements a thread, 256 threads a workgroup
-    return (int64_t)a.B * a.heads <= limit && (int64_t)a.B * a.kv_heads * (rows > a.Lk ? rows : a.Lk) <= limit * 4;
+    // Rows of a key head are counted in 32 bits, and so are the threads of a launch: 256 per 128 rows of a key head's longer side, 512 per
+    // key head where a side is short.  (Splits add at most 2304 workgroups: nine fit on each of 256 compute units.)
+    const int64_t rows = (int64_t)(a.heads / a.kv_heads) * a.Lq, side = rows > a.Lk ? rows : a.Lk, groups = (int64_t)a.B * a.kv_heads;
+    const int64_t limit = ((int64_t)1 << 32) / 512 - 4096;
+    return side <= (int64_t)1 << 30 && groups <= limit && (side + 127) / 128 <= 2 * limit / (groups > 0 ? groups : 1);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -7,9 +7,10 @@ import torch
 import torch.autograd.forward_ad as fwad
 
 from rlipv2_amd import _lib
+from rlipv2_amd.attention import cross_attention
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from attention_reference import BACK, HEAD, NO_WORK  # noqa: E402
+from attention_reference import BACK, HEAD, NO_WORK, WORK  # noqa: E402
 
 
 @pytest.mark.parametrize("which", [0, 1, 2])
@@ -36,3 +37,19 @@ def test_workspaces_do_not_grow_with_the_product_of_the_lengths(dtype, B, Lq, Lk
         head = HEAD.pack(dtype, B, H, Hk, Lq, Lk, D, 1.0, 1.0, 0, 16, 16, 16, *(0,) * 9, 0, 0, 0, 0, 16, 0, 16)
         need = L.cross_attention_workspace_bytes(head + BACK.pack(16, 0, 0, 0, 16, 16, 16, 16) + NO_WORK, backward)
         assert need <= 256 * 9 * 128 * 2 * 256 * 4 + B * H * Lq * 8, need
+
+
+def _entries(**change):
+    """what the two C entries say to a call (addresses that nothing may touch: it must end in the checks)"""
+    a = {**dict(dtype=_lib.MSDA_BF16, B=1, H=4, Hk=4, Lq=4, Lk=4, D=8, scale=1.0), **change}
+    st = (a["Lq"] * 32, 32, 8)
+    head = HEAD.pack(a["dtype"], a["B"], a["H"], a["Hk"], a["Lq"], a["Lk"], a["D"], a["scale"], 1.0, 0, 4096, 4096, 4096, *st, *st, *st, 0, 0, 0, 0,
+                     4096, 0, 4096)
+    args = head + BACK.pack(4096, *st, 4096, 4096, 4096, 4096) + WORK.pack(4096, 1 << 40)
+    L = _lib.lib()
+    return L.cross_attention_forward(args, None), L.cross_attention_backward(args, None), L.cross_attention_supported(args)
+
+
+@pytest.mark.parametrize("change", [{"Lq": 1 << 30}, {"Lk": 1 << 30}, {"B": 1 << 23}, {"B": 1 << 14, "Lq": 1 << 15}], ids=str)
+def test_launches_of_more_threads_than_32_bits_count_are_refused(change):
+    assert _entries(**change) == (-2, -2, 0)
