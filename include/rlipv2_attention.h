@@ -17,7 +17,7 @@
  *   delta    [B, heads, Lq] float32: scratch of the backward call
  *
  * A row without a key that counts gives zeros, and no gradient.  Keys and values that do not count are never multiplied with:
- * their NaNs and infinities stay where they are, their gradients are zero.  scale > 0.
+ * their NaNs and infinities stay where they are, their gradients are zero.  scale >= 1e-30 and finite.
  * Supported: D a multiple of 8 up to 256, heads a multiple of kv_heads, dtype MSDA_BF16 or MSDA_F32.  Results do not depend on
  * anything but the operands (no atomics: repeated calls give the same bits).  Nothing allocates or synchronises; work is enqueued
  * on `stream`.  Return value: 0 or an msda_status code (rlipv2_msda.h). */

@@ -24,7 +24,7 @@ def cross_attention(query, key, value, key_padding_mask=None, key_lengths=None, 
     key_padding_mask [B, Lk] bool: True marks keys that do not count (as `NestedTensor.mask`); key_lengths [B] int32: only the
     first ones count.  Both may be given.  Masked keys and values are never multiplied with (a NaN there stays there) and get
     zero gradients; a query without any key gives zeros.
-    scale: positive, 1 / sqrt(D) by default.  keep [B, H, Lq, Lk] bool or uint8: dropout mask of the probabilities, kept ones are
+    scale: 1e-30 to 1e30, 1 / sqrt(D) by default.  keep [B, H, Lq, Lk] bool or uint8: dropout mask of the probabilities, kept ones are
     multiplied by `keep_scale`.
     Sums, maxima and gradients are accumulated in float32; calls are repeatable bit for bit.  Differentiable (once, in
     reverse mode) in query, key and value; capturable in a HIP graph."""
@@ -45,8 +45,8 @@ def cross_attention(query, key, value, key_padding_mask=None, key_lengths=None, 
     if scale is None:
         scale = D ** -0.5
     scale, keep_scale = float(scale), float(keep_scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"cross_attention: scale must be positive and finite (got {scale})")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"cross_attention: scale must lie between 1e-30 and 1e30 (got {scale})")
     if key_padding_mask is not None:
         if key_padding_mask.dtype != torch.bool or key_padding_mask.shape != (B, Lk):
             raise ValueError(f"cross_attention: key_padding_mask must be a bool tensor [{B}, {Lk}], True where a key does not count")

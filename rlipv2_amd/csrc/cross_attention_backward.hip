@@ -510,11 +510,14 @@ bool sizes_ok(const cross_attention_args &a)
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// (1 / (scale log2 e) times a row's logarithm stays finite: the key pass starts its logits from there)
+bool scale_ok(const cross_attention_args &a) { return a.scale >= 0.99e-30f && a.scale < kInf; }
+
 int check(const cross_attention_args *a, bool backward)
 {
     if (!a) return MSDA_ERR_NULL_POINTER;
     if (a->dtype != MSDA_BF16 && a->dtype != MSDA_F32) return MSDA_ERR_BAD_DTYPE;
-    if (!sizes_ok(*a) || !(a->scale > 0.f) || !(a->scale < kInf)) return MSDA_ERR_BAD_SHAPE;
+    if (!sizes_ok(*a) || !scale_ok(*a)) return MSDA_ERR_BAD_SHAPE;
     if (a->B == 0 || (a->Lq == 0 && (!backward || a->Lk == 0))) return MSDA_OK;
     const void *need[] = {a->query, a->out};
     if (a->Lq > 0)
@@ -551,7 +554,7 @@ extern "C" size_t cross_attention_args_bytes(void) { return sizeof(cross_attenti
 
 extern "C" int cross_attention_supported(const cross_attention_args *a)
 {
-    return a && (a->dtype == MSDA_BF16 || a->dtype == MSDA_F32) && xattn::sizes_ok(*a) && a->scale > 0.f && a->scale < kInf;
+    return a && (a->dtype == MSDA_BF16 || a->dtype == MSDA_F32) && xattn::sizes_ok(*a) && xattn::scale_ok(*a);
 }
 
 extern "C" int cross_attention_short_keys(const cross_attention_args *a) { return cross_attention_supported(a) && xattn::short_side(*a) == 1; }

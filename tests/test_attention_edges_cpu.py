@@ -53,3 +53,16 @@ def _entries(**change):
 @pytest.mark.parametrize("change", [{"Lq": 1 << 30}, {"Lk": 1 << 30}, {"B": 1 << 23}, {"B": 1 << 14, "Lq": 1 << 15}], ids=str)
 def test_launches_of_more_threads_than_32_bits_count_are_refused(change):
     assert _entries(**change) == (-2, -2, 0)
+
+
+@pytest.mark.parametrize("dtype", [_lib.MSDA_BF16, _lib.MSDA_F32])
+def test_a_scale_whose_reciprocal_overflows_is_refused(dtype):
+    """the backward pass starts its logits from -L / (scale log2 e)"""
+    for scale in (1e-31, 1e-38, 1e-45):
+        assert _entries(dtype=dtype, scale=scale) == (-2, -2, 0)
+    q, k = torch.zeros(1, 3, 2, 8), torch.zeros(1, 3, 2, 8)
+    for scale in (1e-31, 1e-50, 1e39):
+        with pytest.raises(ValueError, match="scale"):
+            cross_attention(q, k, k, scale=scale)
+    with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
+        cross_attention(q, k, k, scale=1e-30)
