@@ -103,8 +103,12 @@ __global__ __launch_bounds__(kBlock) void generic_backward_kernel(
     const T *__restrict__ loc, const T *__restrict__ aw, const VT *__restrict__ grad_out, int N, int S, int M,
     int D, int L, int Lq, int P, T *__restrict__ g_value, T *__restrict__ g_loc, T *__restrict__ g_aw, int run)
 {
-    // run: consecutive queries of one head that a wave takes (1, or Lq where queries are few: then every address of grad_value
-    // is added to by ONE thread, in the order of the queries, and repeated calls give the same bits)
+    // run: consecutive queries of one head that a wave takes: 1.  float64, the type of gradient checks, with one or two queries: both, so
+    // that every address of grad_value is added to by ONE thread, in the order of the queries, and repeated calls give the same bits (a
+    // check against differences compares them).  It costs waves -- 2 queries of 2 heads of 2048: 389 -> 652 us; 16 queries of 8 heads of
+    // 64, batch 4: 32 -> 384 us, so more queries are left alone.
+    constexpr bool REPEATABLE = sizeof(T) == 8;
+    if (!REPEATABLE) run = 1;
     const int lane = threadIdx.x & 63;
     const long wave = (long)blockIdx.x * kWavesPerBlock + (threadIdx.x >> 6);
     const long nwaves = (long)gridDim.x * kWavesPerBlock;
@@ -115,7 +119,7 @@ __global__ __launch_bounds__(kBlock) void generic_backward_kernel(
         const long task = at / run;
         const int m = (int)(task % M);
         const long n = task / ((long)runs * M);
-        const long qm = (n * Lq + (task / M) % runs * run + at % run) * M + m;
+        const long qm = REPEATABLE ? (n * Lq + (task / M) % runs * run + at % run) * M + m : at;
         const T *lp = loc + qm * L * P * 2;
         const T *wp = aw + qm * L * P;
         const long img = n * S * row + (long)m * D;
@@ -177,7 +181,7 @@ template <typename T, typename VT> void fwd(const Problem &p)
 }
 template <typename T, typename VT> void bwd(const Problem &p)
 {
-    const int run = p.Lq <= 16 ? p.Lq : 1;
+    const int run = sizeof(T) == 8 && p.Lq <= 2 ? p.Lq : 1;
     const long total = (long)p.N * p.Lq * p.M / run;
     hipLaunchKernelGGL((generic_backward_kernel<T, VT>), dim3(grid_for(total)), dim3(kBlock), 0, p.stream,
                        (const VT *)p.value, p.shapes, p.starts, (const T *)p.loc, (const T *)p.aw,
