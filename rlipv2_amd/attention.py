@@ -26,7 +26,9 @@ def cross_attention(query, key, value, key_padding_mask=None, key_lengths=None, 
     zero gradients; a query without any key gives zeros.
     scale: 1e-30 to 1e30, 1 / sqrt(D) by default.  keep [B, H, Lq, Lk] bool or uint8: dropout mask of the probabilities, kept ones are
     multiplied by `keep_scale`.
-    Sums, maxima and gradients are accumulated in float32; calls are repeatable bit for bit.  Differentiable (once, in
+    Sums, maxima and gradients are accumulated in float32; calls are repeatable bit for bit.  bfloat16 rounds the probabilities, and in
+    the backward pass of calls of more than 2^24 of them (batch and heads included) or with `keep` also dS, for the products with them:
+    errors of 1.1 (result) and 1.4 times (those gradients) a rounded exact value's; smaller calls' gradients are at 1.0.  Differentiable (once, in
     reverse mode) in query, key and value; capturable in a HIP graph."""
     for name, t in (("query", query), ("key", key), ("value", value)):
         if not isinstance(t, torch.Tensor) or t.dim() != 4:

@@ -498,9 +498,13 @@ inline int tile_lds(const cross_attention_args &a) { return rows_per_tile(row_by
 inline int least_tiles(const cross_attention_args &a) { return a.dtype == MSDA_BF16 ? 4 : 1; }
 
 // bf16 backward: the products with P and dS also take what the rounding of the two left out (rest_operand).  Without it the gradients'
-// errors are 1.4 times those of rounded exact gradients, and 1.5 to 1.7 times where a few probabilities decide a sum, which small calls do
-// not average out.  It costs a third to a half more matrix instructions: 777 rows over 1091 keys, 8 heads of 128: 82 -> 90 us; 2048 rows
-// over 4096 keys, 16 heads of 128, batch 4: 1270 -> 1650 us.  So calls of few probabilities take it; dropout's own noise is far above it.
+// errors are 1.42 times those of rounded exact gradients, at every size (300 rows over 300 keys to 2048 over 4096: 1.41 to 1.48; with it
+// 1.00 to 1.04): the two roundings weigh as much as the result's own.  It costs matrix instructions only, which calls of few probabilities do
+// not wait for -- step without / with: 300 rows over 300 keys, 8 heads of 64, batch 16 73 / 73 us; 777 over 1091, 8 heads of 128 86 / 91;
+// 1500 over 1500, 8 heads of 64 88 / 85 -- and large ones do: 512 over 512, 16 heads of 128, batch 64 881 / 1077; 2048 over 4096, 16 heads of
+// 128, batch 4 1228 / 1617.  So the rule is the call's whole number of probabilities, batch and heads included: a sequence can get the
+// one or the other with its batch, as it gets other splits.  Not with a dropout mask: dropping with probability 0.1 gives every term of
+// the sums a relative deviation of sqrt(0.1 / 0.9) = 0.33, 170 times a rounding's 2^-9.
 inline bool few_probabilities(const cross_attention_args &a)
 {
     return a.dtype == MSDA_BF16 && !a.keep && (double)a.B * a.heads * a.Lq * a.Lk <= 1 << 24;
