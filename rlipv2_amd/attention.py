@@ -87,6 +87,8 @@ class CrossAttention(nn.Module):
             raise ValueError(f"{num_heads} query heads cannot share {self.num_kv_heads} key heads")
         if head_dim is None and self.head_dim * num_heads != embed_dim:
             raise ValueError(f"embed_dim {embed_dim} is not divisible by num_heads {num_heads}")
+        if not 0.0 <= dropout < 1.0:
+            raise ValueError(f"dropout must be at least 0 and below 1 (got {dropout})")
         states_dim = embed_dim if states_dim is None else states_dim
         self.dropout = dropout
         self.q_proj = nn.Linear(embed_dim, num_heads * self.head_dim, bias=bias)

@@ -7,7 +7,7 @@ import torch
 import torch.autograd.forward_ad as fwad
 
 from rlipv2_amd import _lib
-from rlipv2_amd.attention import cross_attention
+from rlipv2_amd.attention import CrossAttention, cross_attention
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from attention_reference import BACK, HEAD, NO_WORK, WORK  # noqa: E402
@@ -66,3 +66,11 @@ def test_a_scale_whose_reciprocal_overflows_is_refused(dtype):
             cross_attention(q, k, k, scale=scale)
     with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
         cross_attention(q, k, k, scale=1e-30)
+
+
+def test_module_refuses_a_dropout_that_keeps_nothing():
+    """(kept probabilities are divided by 1 - dropout)"""
+    for p in (1.0, -0.1, 1.5, float("nan")):
+        with pytest.raises(ValueError, match="dropout"):
+            CrossAttention(64, 4, dropout=p)
+    assert CrossAttention(64, 4, dropout=0.999).dropout == 0.999
