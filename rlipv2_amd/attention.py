@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from . import _lib
+from . import _lib, roofline
 
 _DTYPES = (torch.float32, torch.bfloat16)
 
@@ -68,7 +68,13 @@ def cross_attention(query, key, value, key_padding_mask=None, key_lengths=None, 
             raise RuntimeError(f"cross_attention: {name} must be on the query's device")
     if not query.is_cuda:
         raise RuntimeError("Not implemented on the CPU")
-    return _lib.operators().cross_attention(query, key, value, key_padding_mask, key_lengths, keep, scale, keep_scale)
+    out = _lib.operators().cross_attention(query, key, value, key_padding_mask, key_lengths, keep, scale, keep_scale)
+    if roofline.active:
+        # (the backward node is C++ and reports nothing: its operands are added here, where it will run)
+        moved = roofline.tensor_bytes(query, key, value, key_padding_mask, key_lengths, keep, out)
+        again = roofline.tensor_bytes(query, key, value, out) if out.requires_grad else 0
+        roofline.add(moved + (moved + again if again else 0), (14 if again else 4) * B * H * Lq * Lk * D)
+    return out
 
 
 class CrossAttention(nn.Module):

@@ -284,6 +284,8 @@ class GradientClipper:
             raise ValueError(f"grad_scale must be positive and finite (got {grad_scale})")
 
     def _norm(self, norm_type, grad_scale):
+        if roofline.active:
+            roofline.add(roofline.tensor_bytes(*self.tensors))
         return _lib.operators().grad_norm(*self._src, self._numel, len(self.tensors), _ORDERS[float(norm_type)], grad_scale, self.device.index)
 
     def norm(self, norm_type=2.0, grad_scale=1.0):
@@ -308,6 +310,8 @@ class GradientClipper:
         if error_if_nonfinite and not bool(torch.isfinite(norm)):
             raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients is non-finite, so it cannot be clipped.")
         _lib.operators().grad_clip(*self._src, *self._dst, self._numel, len(self.tensors), max_norm, grad_scale, work)
+        if roofline.active:
+            roofline.add(roofline.tensor_bytes(*self.tensors, *(self.tensors if self.out is None else self.out)))
         torch.autograd.graph.increment_version(self.tensors if self.out is None else self.out)
         return norm
 
