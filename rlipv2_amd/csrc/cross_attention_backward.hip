@@ -569,6 +569,7 @@ extern "C" int cross_attention_forward(const cross_attention_args *a, void *stre
 {
     if (const int st = xattn::check(a, false)) return st;
     if (a->B == 0 || a->Lq == 0) return MSDA_OK;
+    (void)hipGetLastError();                  // (an error that an earlier call left is not this one's)
     return xattn::forward(*a, static_cast<hipStream_t>(stream));
 }
 
@@ -576,5 +577,6 @@ extern "C" int cross_attention_backward(const cross_attention_args *a, void *str
 {
     if (const int st = xattn::check(a, true)) return st;
     if (a->B == 0 || (a->Lq == 0 && a->Lk == 0)) return MSDA_OK;
+    (void)hipGetLastError();                  // (an error that an earlier call left is not this one's)
     return xattn::backward(*a, static_cast<hipStream_t>(stream));
 }

@@ -300,6 +300,7 @@ extern "C" int grad_norm(const void *const *src, const uint8_t *src_types, const
     if (!workspace || !norm || workspace_bytes < grad_norm_workspace_bytes(n)) return MSDA_ERR_NULL_POINTER;
     if (reinterpret_cast<uintptr_t>(workspace) % 8) return MSDA_ERR_ALIGNMENT;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
+    (void)hipGetLastError();                  // (an error that an earlier call left is not this one's)
     double *joined = static_cast<double *>(workspace), *partial = joined + 1;
     const int64_t chunk = chunk_of(total);
     NormList list;
@@ -343,6 +344,7 @@ extern "C" int grad_clip(const void *const *src, const uint8_t *src_types, void 
     if (!workspace) return MSDA_ERR_NULL_POINTER;
     if (reinterpret_cast<uintptr_t>(workspace) % 8) return MSDA_ERR_ALIGNMENT;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
+    (void)hipGetLastError();                  // (an error that an earlier call left is not this one's)
     const double *joined = static_cast<const double *>(workspace);
     const int64_t chunk = chunk_of(total);
     ClipList list;
