@@ -10,11 +10,13 @@
 // rounded to the operands' type for the products (relative 2^-9 in bf16), everything else is float32.  delta is taken from out and what
 // its rounding took (out_low): with the rounded out alone the errors of dQ and dK grow from 2.4e-3 to 2.7e-3 over 64 keys.
 //
-// What bounds it, measured (bf16): 2048 rows over 4096 keys, 16 heads of 128, batch 4: query_kernel 435 us (950 TFLOP/s), key_kernel 610 us
-// (900 TFLOP/s): matrix instructions and the vector work between them, two waves per SIMD; the key pass holds 192 registers of operands
+// What bounds it, measured (bf16; averages of 20 calls in a kernel trace, profiles/operators_kernel_stats.csv, and the last of them, the
+// clock settled): 2048 rows over 4096 keys, 16 heads of 128, batch 4: query_kernel 425 us (406: 1015 TFLOP/s), key_kernel 606 us (561: 980
+// TFLOP/s): matrix instructions and the vector work between them, two waves per SIMD; the key pass holds 192 registers of operands
 // and sums.  Read ahead of the matrix instructions: key pass 1107 -> 920 us, row statistics as the accumulators' start values and no
-// dropout code: -> 610.  777 rows of 12 heads of 64 over 1091 keys, batch 3: 30 + 35 us, short loops between prologue and epilogue.
-// float32: 80 TFLOP/s, heads of 256 58 (registers).
+// dropout code: -> 610.  777 rows of 12 heads of 64 over 1091 keys, batch 3: 30 + 34 us, short loops between prologue and epilogue.
+// float32, the same 2048 rows: 127 TFLOP/s; heads of 256, 5000 rows over 5000 keys: 87, with the logits a second time for the keys'
+// gradient (registers).
 #include "cross_attention_device.h"
 
 namespace {

@@ -13,14 +13,16 @@
 // Few query rows: the keys are cut into splits (plan_for), each writes its normalised float32 result and its logarithm of the sum, and
 // combine_kernel joins them in the order of the splits.
 //
-// What bounds it, measured (bf16, this kernel with its joining): one token of eight requests, four heads of 128 per key head, 22 223 keys
-// 128 us (569 MB: 4.4 TB/s, HBM); 64 rows of 8 heads of 256 over 22 223 keys, batch 4, 147 us (590 MB: 4.0 TB/s); 22 223 rows over 64 keys,
-// heads of 256, 176 us (728 MB: 4.1 TB/s, HBM); 300 rows over 22 223 keys, heads of 32, 92 us (32 exponentials, 96 other vector and 8
-// matrix instructions per wave and tile: vector issue, and 384 rows for 300); 2048 rows over 4096 keys, 16 heads of 128, batch 4, 302 us
-// (910 TFLOP/s; a large library product reaches 1210 on this card): matrix and vector instructions of two waves per SIMD in turn.
+// What bounds it, measured (bf16; this kernel's averages of 20 calls in a kernel trace, profiles/operators_kernel_stats.csv; under long
+// matrix work the clock settles, the last calls are 7 % faster): one token of eight requests, four heads of 128 per key head, 22 223 keys
+// 131 us (569 MB: 4.3 TB/s, HBM); 64 rows of 8 heads of 256 over 22 223 keys, batch 4, 166 us (590 MB: 3.6 TB/s); 22 223 rows over 64 keys,
+// heads of 256, 187 us (728 MB: 3.9 TB/s, HBM); 300 rows over 22 223 keys, heads of 32, 87 us (32 exponentials, 96 other vector and 8
+// matrix instructions per wave and tile: vector issue; 384 rows for 300, two of a last workgroup's four waves without any); 2048 rows over 4096 keys, 16
+// heads of 128, batch 4, 327 us (840 TFLOP/s; 304 us, 905 in the last calls; a large library product reaches 1210 on this card): matrix and
+// vector instructions of two waves per SIMD in turn.
 // The copies' wait in front of the loop instead of inside it: single tokens 683 -> 144 us; reads ahead of the matrix instructions and
-// copies with scalar bases: the 2048 rows 451 -> 350 us; variants without the dropout mask: -> 302 us.  float32: 94 TFLOP/s (library
-// product 154).
+// copies with scalar bases: the 2048 rows 451 -> 350 us; variants without the dropout mask: -> 302 us (timed without the trace).  float32 at the
+// same size 2114 us, 130 TFLOP/s (library product 154); heads of 256, 5000 rows over 5000 keys: 92.
 #include "cross_attention_device.h"
 
 namespace {

