@@ -16,7 +16,8 @@
  *            call, read by the backward call; may be NULL in a forward call)
  *   delta    [B, heads, Lq] float32: scratch of the backward call
  *
- * A row without a key that counts gives zeros, and no gradient.  Keys and values that do not count are never multiplied with:
+ * A row without a key that counts gives zeros, and no gradient.  Where lengths or Lk leave one key, the gradients of query and key are
+ * exactly zero.  Keys and values that do not count are never multiplied with:
  * their NaNs and infinities stay where they are, their gradients are zero.  scale >= 1e-30 and finite.
  * Supported: D a multiple of 8 up to 256, heads a multiple of kv_heads, dtype MSDA_BF16 or MSDA_F32.  Results do not depend on
  * anything but the operands (no atomics: repeated calls give the same bits).  Nothing allocates or synchronises; work is enqueued

@@ -168,6 +168,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void query_kernel(cross_attention_arg
     float *part = static_cast<float *>(a.workspace) + (int64_t)sp * a.B * a.Lq * a.heads * a.D;
     if (sizeof(T) == 4 && stretch.index > 0 && ok) add_row(acc, (splits == 1 ? static_cast<const float *>(a.grad_query) : part) + dense, 1.f, a.D, half);
     const float factor = sizeof(T) == 4 && stretch.index + 1 < stretch.count ? 1.f : a.scale;
+    zero_unless(!mask.one(), acc);
     __syncthreads();                          // everybody is done with the tiles: their memory carries the results out
     constexpr int REGION = 2 * BUF / NW;
     char *region = lds + wave * REGION;
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void key_kernel(cross_attention_args 
     const float factor = sizeof(T) == 4 && stretch.index + 1 < stretch.count ? 1.f : a.scale;
     // (a key that does not count has P = 0, but 0 times an infinite or NaN grad_out is NaN)
     if constexpr (DV) zero_unless(counts, dv);
-    if constexpr (DK) zero_unless(counts, dk);
+    if constexpr (DK) zero_unless(counts && !mask.one(), dk);
     __syncthreads();                          // everybody is done with the tiles: their memory carries the results out
     constexpr int REGION = 2 * BUF / NW;
     char *region = lds + wave * REGION;

@@ -338,6 +338,8 @@ struct KeyMask {
         padding = a.padding ? static_cast<const uint8_t *>(a.padding) + (int64_t)b * a.padding_stride : nullptr;
         length = a.lengths ? max(0, min(a.Lk, static_cast<const int *>(a.lengths)[b])) : a.Lk;
     }
+    // A softmax over one key does not depend on the query: dS is 0, where P (dP - delta) is what the two sums' orders leave.
+    __device__ __forceinline__ bool one() const { return length == 1; }
     // (the byte is loaded a tile ahead of the ballot that needs it)
     __device__ __forceinline__ int load(int key) const { return key < length ? (padding ? (int)padding[key] : 0) : 1; }
 };

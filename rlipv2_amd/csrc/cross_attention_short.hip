@@ -372,6 +372,7 @@ __global__ __launch_bounds__(2 * DP, 2) void short_kernel(cross_attention_args a
                 XATTN_SCHED_GROUP(0x8, M - STEPS);
             }
         }
+        if (mask.one()) clear(long1);
         if (!FEW_KEYS && word != ~0u) {        // (keys that do not count: 0 times an infinite or NaN grad_out is NaN)
             zero_unless((word >> (lane & 31)) & 1, long1);
             zero_unless((word >> (lane & 31)) & 1, long2);
@@ -410,7 +411,7 @@ __global__ __launch_bounds__(2 * DP, 2) void short_kernel(cross_attention_args a
             dense = (((int64_t)b * a.Lq + q) * a.heads + hk * G + g) * a.D;
         }
         f32x16 v[1] = {sum1[i]};
-        if (FEW_KEYS) zero_unless((keys >> r) & 1, v);
+        zero_unless(!mask.one() && (!FEW_KEYS || ((keys >> r) & 1)), v);
         T *first = static_cast<T *>(FEW_KEYS ? a.grad_key : a.grad_query) + d0;
         if (splits == 1) put_rows<T, 32, OUT_REGION>(v, a.scale, mine, first, dense, a.D - d0, lane);
         else put_rows<float, 32, OUT_REGION>(v, 1.f, mine, partial, dense, a.D - d0, lane);

@@ -45,3 +45,25 @@ def test_delta_does_not_carry_the_rounding_of_the_result(lib, case, states):  # 
     """also where only the query is trained"""
     x = inputs(case)
     check_grad_query(run(lib, x, 0.3, states)["grad_query"], x, 0.3)
+
+
+ONE_KEY = [(2, 40, 1, 2, 1, 32, False), (2, 70, 1, 2, 1, 128, False), (1, 40, 1, 1, 1, 256, True)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("case", ONE_KEY, ids=str)
+def test_one_key_leaves_no_gradient_for_query_and_key(lib, case, dtype):  # noqa: F811
+    """dS = P (dP - delta) is 0 where P = 1, not what the two sums' orders leave of it"""
+    x = make(*case[:6], dtype, "", case[6], seed=5)
+    got = run(lib, x, 0.3)
+    assert not bool(got["grad_query"].any()) and not bool(got["grad_key"].any()) and bool(got["grad_value"].any())
+
+
+@pytest.mark.parametrize("case", [(2, 40, 90, 2, 1, 32), (2, 70, 40, 2, 1, 128), (2, 20, 100, 2, 1, 128)], ids=str)
+def test_a_sequence_whose_length_is_one(lib, case):  # noqa: F811
+    x = make(*case, torch.bfloat16, "", seed=6)
+    x["lengths"] = torch.tensor([case[2], 1], dtype=torch.int32)
+    got = run(lib, x, 0.3)
+    for name in ("grad_query", "grad_key"):
+        assert not bool(got[name][1].any()) and bool(got[name][0].any())
+    assert bool(got["grad_value"][1, 0].any())

@@ -137,3 +137,17 @@ def test_float32_rows_whose_maximum_grows_from_stretch_to_stretch():
     x["dead"] = x["padding"]
     got = dict(zip(("out", "grad_query", "grad_key", "grad_value"), run(x, 0.25)))
     check(got, reference(x["q"], x["k"], x["v"], x["g"], x["dead"], 0.25))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("case", [(2, 300, 1, 4, 2, 32), (3, 3000, 1, 2, 2, 128), (1, 40, 1, 1, 1, 256), (2, 700, 900, 2, 1, 64), (2, 3000, 40, 2, 1, 128),
+                                  (2, 20, 5000, 2, 1, 128), (1, 5000, 1, 300, 300, 128)], ids=str)
+def test_one_key_leaves_no_gradient_for_query_and_key(case, dtype):
+    """dS = P (dP - delta) is 0 where P = 1, not what the two sums' orders leave of it; the last sequence, or all"""
+    x = make(*case, dtype, "", seed=5, device=DEV)
+    x["lengths"] = torch.full((case[0],), case[2], dtype=torch.int32, device=DEV)
+    x["lengths"][-1] = 1
+    x["dead"] = torch.arange(case[2], device=DEV)[None] >= x["lengths"][:, None]
+    got = dict(zip(("out", "grad_query", "grad_key", "grad_value"), run(x, 0.3)))
+    check(got, reference(x["q"], x["k"], x["v"], x["g"], x["dead"], 0.3))
+    assert not bool(got["grad_query"][-1].any()) and not bool(got["grad_key"][-1].any()) and bool(got["grad_value"][-1, 0].any())
